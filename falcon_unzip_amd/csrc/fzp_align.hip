@@ -907,7 +907,8 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
 //   * moves are collected in a 32-bit shift register (first step of the block ends up in the highest used bit); its bit 0 is the block's last
 //     move, so the steps do not keep a "previous move" register up to date (one SALU less per step: the scalar port has no slack, see HISTORY.md section 14).
 // The store offset is the step counter: it enters 16 * steps below 2^31 and the signed overflow of its increment ends the block.
-// No DPP source is written fewer than two instructions before it is read (gfx9 DPP hazard).
+// Waits (the compiler does not look into inline asm): between a VALU's write of an SGPR or vcc and a VALU's read of it lie two instructions -- hence the subtraction and the move
+// register's shift between the bases' compare and the select --, between a write of a VGPR and its use through DPP two, and one before v_readlane.
 #define SWB_DPP_SHL " wave_shl:1 row_mask:0xf bank_mask:0xf bound_ctrl:0"
 #define SWB_DPP_SHR " wave_shr:1 row_mask:0xf bank_mask:0xf bound_ctrl:0"
 // one DOWN step.  HC: operand holding H of the previous step; XC: operand holding H of two steps ago, receives the new H;
@@ -922,12 +923,12 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
     "v_writelane_b32 %[qc], s56, " LN "\n\t"                                                      \
     "v_cmp_eq_i32_e64 s[62:63], %[mm], " HC "\n\t"                                                \
     "v_cmp_eq_u32_e32 vcc, %[qc], %[tc]\n\t"                                                      \
+    "v_subrev_u32_e32 %[mm], %[gap], %[mm]\n\t"                                                   \
+    "s_lshl1_add_u32 %[mv], %[mv], 1\n\t"                                                         \
     "v_cndmask_b32_e32 %[sc], %[vmis], %[vmat], vcc\n\t"                                          \
     HDADD "\n\t"                                                                                  \
-    "v_subrev_u32_e32 %[mm], %[gap], %[mm]\n\t"                                                   \
     "v_max_i32_e32 " XC ", %[hd], %[mm]\n\t"                                                      \
     "v_cmp_eq_i32_e64 s[60:61], " XC ", %[hd]\n\t"                                                \
-    "s_lshl1_add_u32 %[mv], %[mv], 1\n\t"                                                         \
     KB                                                      \
     "v_readlane_b32 %[top], " XC ", 0\n\t"                                                        \
     ST                                                                                            \
@@ -946,12 +947,12 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
     "v_writelane_b32 %[tc], s56, 0\n\t"                                                           \
     "v_cmp_eq_i32_e64 s[62:63], %[mm], " HC "\n\t"                                                \
     "v_cmp_eq_u32_e32 vcc, %[qc], %[tc]\n\t"                                                      \
+    "v_subrev_u32_e32 %[mm], %[gap], %[mm]\n\t"                                                   \
+    "s_lshl_b32 %[mv], %[mv], 1\n\t"                                                              \
     "v_cndmask_b32_e32 %[sc], %[vmis], %[vmat], vcc\n\t"                                          \
     HDADD "\n\t"                                                                                  \
-    "v_subrev_u32_e32 %[mm], %[gap], %[mm]\n\t"                                                   \
     "v_max_i32_e32 " XC ", %[hd], %[mm]\n\t"                                                      \
     "v_cmp_eq_i32_e64 s[60:61], " XC ", %[hd]\n\t"                                                \
-    "s_lshl_b32 %[mv], %[mv], 1\n\t"                                                              \
     KB                                                      \
     "v_readlane_b32 %[top], " XC ", 0\n\t"                                                        \
     ST                                                                                            \
