@@ -807,8 +807,8 @@ __device__ __forceinline__ int32_t wave_shl1(int32_t v, int32_t fill) {   // lan
 // "minus infinity" of the spec; that lets the neighbour shifts ride on the add / max / compare
 // themselves (v_add_u32_dpp, v_max_i32_dpp; G = (A >= B) is read off as max(A,B) == A) instead of separate moves.
 // Trace-back masks per step: D = (H == diag + s), G = (A >= B) ("the gap comes from the same lane"), each a
-// 64-bit lane mask; a step's pair is 16 B, stored step-major through the scalar cache.  Upcoming read / contig
-// bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
+// 64-bit lane mask; a step's pair is 16 B, stored step-major: by lane 0 in the checked steps, by a lane per
+// step for a whole interior block (up to 512 B in one run).  Upcoming read / contig bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
 // counted loop with no range checks; the first ~130 and last ~64 steps run the checked variant.
 constexpr int32_t SW_BIAS = 1 << 24;   // stands in for the spec's -2^26 (any value far below every real score gives the same masks on
                                        // reachable cells); small enough that (H << 6) + 6 bits stays below 2^31 for scores < 2^24
@@ -832,14 +832,6 @@ struct BaseStream {          // wave-uniform: lives in SGPRs
         return c;
     }
 };
-
-// wave-uniform 16-byte store through the scalar data cache (s_store_dwordx4): the per-step trace-back masks
-// leave the DP kernel this way, off the vector path.  The data SGPRs are read at issue, so they may be reused at
-// once; the kernel ends with s_dcache_wb.
-__device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, uint64_t lo, uint64_t hi) {
-    const __uint128_t v = ((__uint128_t)hi << 64) | lo;
-    asm volatile("s_store_dwordx4 %[v], %[p], %[o]" ::[v] "s"(v), [p] "s"(base), [o] "s"(byte_off) : "memory");
-}
 
 // one DP step of the checked variant (first ~130 and last ~64 steps of a read): plain HIP, sentinels and validity
 // handled explicitly.  The masks of the step are wave ballots.
@@ -867,7 +859,7 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
         const uint64_t gmask = __ballot(m == H);                                                           \
         Hn = max(hd, m - gap);                                                                             \
         const uint64_t dmask = __ballot(Hn == hd);                                                         \
-        if (STORE) { const uint32_t t_ = (uint32_t)__builtin_amdgcn_readfirstlane(t); scalar_store16(tbr, ((t_ >> 6) * (uint32_t)stride + (t_ & 63u)) * 16u, dmask, gmask); } \
+        if (STORE && lane == 0) tbr[(int64_t)(t >> 6) * stride + (t & 63)] = make_ulonglong2(dmask, gmask);    \
         bool upd;                                                                                          \
         int32_t val;                                                                                       \
         {                                                                                                  \
@@ -897,16 +889,19 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
 
 // ---- interior block: up to 32 steps with every lane strictly inside the matrix, hand-scheduled.
 // The block is VALU-issue bound (a SIMD issues one wave64 VALU op per 4 cycles), so the point is the VALU count
-// per step: 12 (v1.5: an interior block holds no border cell, so nothing of it can be the extension's terminal and it keeps no best-cell key), with 9 SALU and one scalar-memory op riding along on their own ports.
+// per step: 12 for the cells (v1.5: an interior block holds no border cell, so nothing of it can be the extension's terminal and it keeps no best-cell key) and one per non-empty
+// mask word (2 at band 32, 4 at band 64), with 9 SALU riding along on their own port.
 //   * H of two steps ago is never copied or shifted: the two registers swap roles every step (hence two code
 //     parities) and the diagonal's lane shift rides on the add (hence a variant per pair of moves): 8 step variants;
-//   * the two trace-back masks of a step are the 64-bit results of v_cmp_e64 landing in an SGPR quad that
-//     goes out with one s_store_dwordx4 (16 B per step, step-major) -- no per-lane bit accumulators;
+//   * the two trace-back masks of a step are the 64-bit results of v_cmp_e64 landing in an SGPR quad; v_writelane drops its words into the step's own lane of a VGPR quad (band
+//     32: the upper words are zero and stay so), and behind the block every lane that holds a step stores it: 16 B per lane, the block's records in one run.  No vector-memory
+//     instruction per step, no per-lane bit accumulators that would have to be turned round;
 //   * bases entering the band come from two 64-bit SGPR windows (32 bases each, enough for a whole block):
 //     s_bfe_u64 picks the next one, v_writelane drops it into lane 63 (DOWN) / lane 0 (RIGHT);
 //   * moves are collected in a 32-bit shift register (first step of the block ends up in the highest used bit); its bit 0 is the block's last
 //     move, so the steps do not keep a "previous move" register up to date (one SALU less per step: the scalar port has no slack, see HISTORY.md section 14).
-// The store offset is the step counter: it enters 16 * steps below 2^31 and the signed overflow of its increment ends the block.
+// M0 is the step counter and the lane the step's masks go to (a lane select beside an SGPR source can only be M0): it enters as steps - 1, the borrow of its decrement ends the
+// block, so step s of n sits in lane n - 1 - s.  n <= 32: the lanes exist in either band.  M0 comes back as it was.
 // Waits (the compiler does not look into inline asm): between a VALU's write of an SGPR or vcc and a VALU's read of it lie two instructions -- hence the subtraction and the move
 // register's shift between the bases' compare and the select --, between a write of a VGPR and its use through DPP two, and one before v_readlane.
 #define SWB_DPP_SHL " wave_shl:1 row_mask:0xf bank_mask:0xf bound_ctrl:0"
@@ -933,7 +928,7 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
     "v_readlane_b32 %[top], " XC ", 0\n\t"                                                        \
     ST                                                                                            \
     "v_readlane_b32 %[bot], " XC ", " LN "\n\t"                                                   \
-    "s_addk_i32 %[soff], 16\n\t"                                                                  \
+    "s_sub_u32 m0, m0, 1\n\t"                                                                    \
     "s_cbranch_scc1 Lsw%=_end" NP "\n\t"                                                          \
     "s_cmp_gt_i32 %[top], %[bot]\n\t"                                                             \
     "s_cbranch_scc1 Lsw%=_p" NP "DR\n\t"                                                          \
@@ -957,7 +952,7 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
     "v_readlane_b32 %[top], " XC ", 0\n\t"                                                        \
     ST                                                                                            \
     "v_readlane_b32 %[bot], " XC ", " LN "\n\t"                                                   \
-    "s_addk_i32 %[soff], 16\n\t"                                                                  \
+    "s_sub_u32 m0, m0, 1\n\t"                                                                    \
     "s_cbranch_scc1 Lsw%=_end" NP "\n\t"                                                          \
     "s_cmp_gt_i32 %[top], %[bot]\n\t"                                                             \
     "s_cbranch_scc1 Lsw%=_p" NP "RR\n\t"                                                          \
@@ -966,7 +961,8 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
 // the diagonal predecessor of lane k is lane k - 1 + (DOWN moves among the last two) of H(t-2)
 #define SW_BLOCK_ASM(ST, LN)                                                                        \
     asm volatile(                                                                                                                                                                   \
-        "s_nop 1\n\t"                                                                                                                                                               \
+        "s_mov_b32 %[m0s], m0\n\t"                                                                                                                                                  \
+        "s_mov_b32 m0, %[last]\n\t"                                                                                                                                                 \
         "s_cmp_eq_u32 %[dn], 0\n\t"                                                                                                                                                 \
         "s_cbranch_scc1 Lsw%=_enterR\n\t"                                                                                                                                           \
         "s_cmp_eq_u32 %[pm], 0\n\t"                                                                                                                                                 \
@@ -989,24 +985,32 @@ __device__ __forceinline__ void scalar_store16(void *base, uint32_t byte_off, ui
         "v_swap_b32 %[H], %[X]\n"                                                                                                                                                   \
         "Lsw%=_end0:\n\t"                                                                                                                                                           \
         "s_cmp_gt_i32 %[top], %[bot]\n\t"                                                                                                                                           \
-        "s_cselect_b32 %[dn], 0, 1"                                                                                                                                                 \
-        : [H] "+v"(H), [X] "+v"(X), [qc] "+v"(qc), [tc] "+v"(tc), [kb] "+v"(kb), [mv] "+s"(mv), [soff] "+s"(soff),                                                                  \
-          [dn] "+s"(dn), [pm] "+s"(pm), [qsel] "+s"(qsel), [tsel] "+s"(tsel), [hd] "=&v"(hd), [mm] "=&v"(mm), [sc] "=&v"(sc), [top] "=&s"(top), [bot] "=&s"(bot)                    \
-        : [gap] "s"(gapS), [vmat] "v"(vmatS), [vmis] "v"(vmisS), [qb] "s"(qbits), [tb] "s"(tbits), [tbp] "s"(tbp)                                                                   \
-        : "vcc", "scc", "s56", "s57", "s60", "s61", "s62", "s63", "memory");
-#define SWB_STORE "s_store_dwordx4 s[60:63], %[tbp], %[soff]\n\t"
+        "s_cselect_b32 %[dn], 0, 1\n\t"                                                                                                                                             \
+        "s_mov_b32 m0, %[m0s]"                                                                                                                                                      \
+        : [H] "+v"(H), [X] "+v"(X), [qc] "+v"(qc), [tc] "+v"(tc), [kb] "+v"(kb), [mv] "+s"(mv), [dlo] "+v"(rec.x), [dhi] "+v"(rec.y), [glo] "+v"(rec.z), [ghi] "+v"(rec.w),         \
+          [dn] "+s"(dn), [pm] "+s"(pm), [qsel] "+s"(qsel), [tsel] "+s"(tsel), [hd] "=&v"(hd), [mm] "=&v"(mm), [sc] "=&v"(sc), [top] "=&s"(top), [bot] "=&s"(bot), [m0s] "=&s"(m0s)  \
+        : [gap] "s"(gapS), [vmat] "v"(vmatS), [vmis] "v"(vmisS), [qb] "s"(qbits), [tb] "s"(tbits), [last] "s"(last)                                                                 \
+        : "vcc", "scc", "s56", "s57", "s60", "s61", "s62", "s63");
+// a step's masks into its lane of the block's records.  G's words first: D's come from the compare two instructions up, and a VALU's SGPR result may be read by the next VALU two
+// wait states later.
+#define SWB_REC32 "v_writelane_b32 %[glo], s62, m0\n\tv_writelane_b32 %[dlo], s60, m0\n\t"
+#define SWB_REC64 "v_writelane_b32 %[glo], s62, m0\n\tv_writelane_b32 %[ghi], s63, m0\n\tv_writelane_b32 %[dlo], s60, m0\n\tv_writelane_b32 %[dhi], s61, m0\n\t"
+// rec: lane n_steps - 1 - s leaves with the masks of the block's step s (STORE), {D, G} low word first
 template <bool STORE, int BAND>
 __device__ __forceinline__ void sw_block(int32_t &H, int32_t &X, int32_t &qc, int32_t &tc, const uint64_t qbits, const uint64_t tbits, int32_t &kb,
-                                         void *tbp, uint32_t &soff, uint32_t &mv, int32_t &dn, int32_t &pm, const int32_t gapS,
+                                         uint4 &rec, const int32_t n_steps, uint32_t &mv, int32_t &dn, int32_t &pm, const int32_t gapS,
                                          const int32_t vmatS, const int32_t vmisS) {
-    int32_t hd, mm, sc, top, bot;
+    int32_t hd, mm, sc, top, bot, m0s;
+    const int32_t last = n_steps - 1;
     uint32_t qsel = 2u << 16, tsel = 2u << 16;   // s_bfe_u64 operand: width 2, offset 0
     // (the band's last lane enters the asm as a literal: 63, or 31 in the 32-cell band of v1.8 -- there lanes 32..63 of the wave are switched off, and what a DPP shift
     //  would fetch from them reads as zero, which in the biased scores IS "outside the band")
-    if constexpr (BAND == 64) { if constexpr (STORE) { SW_BLOCK_ASM(SWB_STORE, "63") } else { SW_BLOCK_ASM("", "63") } }
-    else { if constexpr (STORE) { SW_BLOCK_ASM(SWB_STORE, "31") } else { SW_BLOCK_ASM("", "31") } }
+    if constexpr (BAND == 64) { if constexpr (STORE) { SW_BLOCK_ASM(SWB_REC64, "63") } else { SW_BLOCK_ASM("", "63") } }
+    else { if constexpr (STORE) { SW_BLOCK_ASM(SWB_REC32, "31") } else { SW_BLOCK_ASM("", "31") } }
 }
 #undef SW_BLOCK_ASM
+#undef SWB_REC32
+#undef SWB_REC64
 #undef SWB_DOWN
 #undef SWB_RIGHT
 #undef SWB_DPP_SHL
@@ -1091,12 +1095,11 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
                 int32_t kb = 0;
                 dn = __builtin_amdgcn_readfirstlane(dn);
                 pm = __builtin_amdgcn_readfirstlane(pm);
-                // the store offset doubles as the block's step counter: it starts 16 * n_steps below 2^31 (the base pointer makes up for
-                // it), and the add that would carry it past 2^31 -- the signed overflow of s_addk_i32 -- ends the block
-                uint32_t soff = 0x80000000u - 16u * (uint32_t)n_steps;
-                const int32_t t_ = __builtin_amdgcn_readfirstlane(t);      // (a block never crosses a multiple of 32 steps: its records are contiguous)
-                void *tbp = (void *)((char *)tbr + (((int64_t)(t_ >> 6) * stride + (t_ & 63)) * 16 - (int64_t)soff));
-                sw_block<STORE, BAND>(H, X, qc, tc, qbits, tbits, kb, tbp, soff, mv, dn, pm, gapS, vmatS, vmisS);
+                uint4 rec = make_uint4(0, 0, 0, 0);
+                sw_block<STORE, BAND>(H, X, qc, tc, qbits, tbits, kb, rec, n_steps, mv, dn, pm, gapS, vmatS, vmisS);
+                // (a block never crosses a multiple of 32 steps: its records are contiguous)
+                if (STORE && lane < n_steps)
+                    tbr[(int64_t)(t >> 6) * stride + (t & 63) + (n_steps - 1 - lane)] = make_ulonglong2(((uint64_t)rec.y << 32) | rec.x, ((uint64_t)rec.w << 32) | rec.z);
                 // (v1.5: no cell of an interior block is a border cell, so the block has no terminal candidates to report)
                 pm = (int32_t)(mv & 1u);                                 // the block's last move (the steps no longer keep it up to date)
                 const int32_t nd = __popc(mv);                          // DOWN moves of the block (mv holds exactly n_steps bits)
@@ -1119,7 +1122,6 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
         }
     }
     if ((t & 63) != 0) SW_FLUSH(true)
-    asm volatile("s_dcache_wb" ::: "memory");   // the masks went through the scalar cache
     // best cell: max score, then earliest step, then lowest lane
     int32_t s_b = bs, t_b = bt < 0 ? 0x7fffffff : bt, l_b = lane;
 #pragma unroll

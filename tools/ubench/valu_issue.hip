@@ -18,7 +18,7 @@
 enum Kind { ADD = 0, MAX, ADD_DPP, MAX_DPP, MOV_DPP, CMP_SGPR, CMP_VCC, CNDMASK, MAX3, READLANE, WRITELANE, PK_ADD_I16, PK_MAX_I16, SW_MIX, SW_MIX_NOLANE, SW_MIX_SEL, CNDMASK_E64, MAX_3REG, N_KINDS };
 static const char *kind_name[N_KINDS] = {"v_add_u32", "v_max_i32", "v_add_u32_dpp(wave_shl)", "v_max_i32_dpp(wave_shr)", "v_mov_b32_dpp(wave_shl)",
                                          "v_cmp_eq_i32_e64->sgpr", "v_cmp_eq_u32_e32->vcc", "v_cndmask_b32 (vcc written once, one asm statement)", "v_max3_i32", "v_readlane_b32",
-                                         "v_writelane_b32", "v_pk_add_i16", "v_pk_max_i16", "k_sw step mix (13 VALU + 9 SALU + s_store)", "k_sw step mix without readlane/writelane", "k_sw step mix, Hnew = cmp_ge + cndmask_e64 (no max + cmp_eq)", "v_cndmask_b32_e64 (sgpr pair mask)", "v_max_i32 (dst apart from both sources)"};
+                                         "v_writelane_b32", "v_pk_add_i16", "v_pk_max_i16", "k_sw step mix (13 VALU + 9 SALU)", "k_sw step mix without readlane/writelane", "k_sw step mix, Hnew = cmp_ge + cndmask_e64 (no max + cmp_eq)", "v_cndmask_b32_e64 (sgpr pair mask)", "v_max_i32 (dst apart from both sources)"};
 
 #define R8(X) X(0) X(1) X(2) X(3) X(4) X(5) X(6) X(7)
 
