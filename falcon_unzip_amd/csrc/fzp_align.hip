@@ -807,8 +807,9 @@ __device__ __forceinline__ int32_t wave_shl1(int32_t v, int32_t fill) {   // lan
 // "minus infinity" of the spec; that lets the neighbour shifts ride on the add / max / compare
 // themselves (v_add_u32_dpp, v_max_i32_dpp; G = (A >= B) is read off as max(A,B) == A) instead of separate moves.
 // Trace-back masks per step: D = (H == diag + s), G = (A >= B) ("the gap comes from the same lane"), each a
-// 64-bit lane mask; a step's pair is 16 B, stored step-major: by lane 0 in the checked steps, by a lane per
-// step for a whole interior block (up to 512 B in one run).  Upcoming read / contig bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
+// 64-bit lane mask; a step's pair is 16 B, stored step-major.  A step's masks are kept in a lane of their own until an interior
+// block, or 32 steps of the checked variant, are through, and leave in one run of up to 512 B (a store per checked step made the bases' next vector load wait for it: the launch
+// of a bench step 0.47 ms instead of 0.36).  Upcoming read / contig bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
 // counted loop with no range checks; the first ~130 and last ~64 steps run the checked variant.
 constexpr int32_t SW_BIAS = 1 << 24;   // stands in for the spec's -2^26 (any value far below every real score gives the same masks on
                                        // reachable cells); small enough that (H << 6) + 6 bits stays below 2^31 for scores < 2^24
@@ -859,7 +860,7 @@ struct BaseStream {          // wave-uniform: lives in SGPRs
         const uint64_t gmask = __ballot(m == H);                                                           \
         Hn = max(hd, m - gap);                                                                             \
         const uint64_t dmask = __ballot(Hn == hd);                                                         \
-        if (STORE && lane == 0) tbr[(int64_t)(t >> 6) * stride + (t & 63)] = make_ulonglong2(dmask, gmask);    \
+        if (STORE) { const bool mine = lane == (t & 31); rd = mine ? dmask : rd; rg = mine ? gmask : rg; }     \
         bool upd;                                                                                          \
         int32_t val;                                                                                       \
         {                                                                                                  \
@@ -885,6 +886,16 @@ struct BaseStream {          // wave-uniform: lives in SGPRs
             if (lane == 0) mvr[(t - 1) >> 6] = make_ulonglong2(mvacc, (uint64_t)(uint32_t)(i0 - __popcll(mvacc))); \
             mvacc = 0;                                                                                     \
         }                                                                                                  \
+    }
+
+// the checked steps t_put .. t - 1 (all of one 32-step block) leave their lanes
+#define SW_PUT()                                                                                           \
+    {                                                                                                      \
+        if (STORE) {                                                                                       \
+            const int32_t s_ = ((t - 1) & ~31) + lane;                                                     \
+            if (s_ >= t_put && s_ < t) tbr[(int64_t)(s_ >> 6) * stride + (s_ & 63)] = make_ulonglong2(rd, rg); \
+        }                                                                                                  \
+        t_put = t;                                                                                         \
     }
 
 // ---- interior block: up to 32 steps with every lane strictly inside the matrix, hand-scheduled.
@@ -1073,6 +1084,8 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
     qs.init(qpk, qb + (HB - 1));
     ts.init(tpk, tbase + (HB + 1));
     bool done = false;
+    uint64_t rd = 0, rg = 0;      // the masks of checked step 32 k + lane, not stored yet
+    int32_t t_put = 0;            // the first step of which that is so
     while (!done) {
         t = __builtin_amdgcn_readfirstlane(t); i0 = __builtin_amdgcn_readfirstlane(i0);
         // how many steps can run with every lane strictly inside the matrix?  Each step advances i0 or
@@ -1080,6 +1093,7 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
         int32_t safe = swb::sw_interior_safe(t, i0, nq, nt, BAND);      // (fzp_swb_core.h: shared with the host test that pins it)
         if (safe > 0) {
             // ---- interior: asm blocks of <= 32 steps
+            if (t > t_put) SW_PUT()
             int32_t qpos_i = i0 + BAND, tpos_i = t - i0;               // next bases to enter at the band's last lane / lane 0
             const int32_t vmatS = match, vmisS = -mismatch;
             const int32_t gapS = __builtin_amdgcn_readfirstlane(gap);
@@ -1111,16 +1125,19 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
             }
             down = dn != 0;
             pdown = pm != 0;
+            t_put = t;      // (the blocks stored their own)
             // back to the checked variant: scalar base streams resume at the current positions
             qpos = i0 + BAND; tpos = t - i0;
             qs.init(qpk, qb + qpos);
             ts.init(tpk, tbase + tpos);
         } else {
             SW_STEP()
+            if ((t & 31) == 0) SW_PUT()
             if ((t & 63) == 0) SW_FLUSH(false)
             if (i0 > nq - 1 || (t - 1) - (i0 + BAND - 1) > nt - 1 || t >= max_steps) done = true;
         }
     }
+    if (t > t_put) SW_PUT()
     if ((t & 63) != 0) SW_FLUSH(true)
     // best cell: max score, then earliest step, then lowest lane
     int32_t s_b = bs, t_b = bt < 0 ? 0x7fffffff : bt, l_b = lane;
@@ -1134,6 +1151,7 @@ __global__ void __launch_bounds__(64) k_sw(const uint64_t *__restrict__ lo_dev, 
 }
 #undef SW_STEP
 #undef SW_FLUSH
+#undef SW_PUT
 
 // ---- K1 hot kernel, bit-sliced form: one READ per lane (64 extensions per wave), the 64 cells of a read's anti-diagonal in the 64 bits of a register
 // pair, the DP values as differences in three bit planes (fzp_swb_core.h: the cell function, checked on the host against the scalar twin).  Same spec,
