@@ -809,7 +809,7 @@ __device__ __forceinline__ int32_t wave_shl1(int32_t v, int32_t fill) {   // lan
 // Trace-back masks per step: D = (H == diag + s), G = (A >= B) ("the gap comes from the same lane"), each a
 // 64-bit lane mask; a step's pair is 16 B, stored step-major.  A step's masks are kept in a lane of their own until an interior
 // block, or 32 steps of the checked variant, are through, and leave in one run of up to 512 B (a store per checked step made the bases' next vector load wait for it: the launch
-// of a bench step 0.47 ms instead of 0.36).  Upcoming read / contig bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
+// of a bench step 0.46 ms instead of 0.37).  Upcoming read / contig bases sit in 64-bit SGPR windows, so no step waits on memory.  The interior of the matrix runs a
 // counted loop with no range checks; the first ~130 and last ~64 steps run the checked variant.
 constexpr int32_t SW_BIAS = 1 << 24;   // stands in for the spec's -2^26 (any value far below every real score gives the same masks on
                                        // reachable cells); small enough that (H << 6) + 6 bits stays below 2^31 for scores < 2^24
